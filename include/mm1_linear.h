@@ -34,7 +34,8 @@ size_t mm1_linear_workspace_size(int M, int N, int K, int x_layout, int w_layout
  * bf16(z), for the backward of an activation (else NULL).  bf16 x and w, fp32 sums and epilogue, one rounding
  * to out's type (fp32, or bf16 where out_f32 = 0).  bias [N] and residual [M, N]
  * may be NULL; *_f32 says their type; ldr, ldp and ldo are the row strides of
- * residual, pre and out (at most 2^24), which lie at any element alignment.
+ * residual, pre and out, which lie at any element alignment: at most 2^24, and
+ * 2^23 for fp32 tensors of more than 64 rows.
  * x and w as in mm1_gemm: MM1_GEMM_ROW or _COL (x ROW with w ROW or COL, or both
  * COL, which takes no activation), strides multiples of 8, 16-byte aligned, but
  * with any M, N and K >= 1 (bounded as in mm1_gemm, K <= 2^28): a row of an operand
@@ -54,7 +55,8 @@ size_t mm1_linear_backward_workspace_size(int M, int N, int K, int dz, int dx, i
  * unless it is NULL: with dz = dy act'(z), z from pre (not read without an
  * activation),
  *   dx [M, K] = dz w,  dw = dz^T x in w's own layout ([N, K] for ROW, [K, N] for
- *   COL; contiguous),  dbias [N] = sum over the rows of dz.
+ *   COL; contiguous),  dbias [N] = sum over the rows of dz.  N and K as mm1_linear's
+ *   strides.
  * dz is fp32; it enters the products rounded to bf16 (dy itself where it is bf16
  * and there is no activation) and dbias as it is.  fp32 sums in a fixed order, one
  * rounding to each result's type.  x [M, K] ROW and w as mm1_linear takes them

@@ -5,6 +5,9 @@
 
 namespace mm1 {
 
+// Rows of a wave's block at most, whose byte offsets the epilogue forms in 32 bits.
+constexpr int EPILOGUE_ROWS = 128;
+
 struct LinearArgs {
   const void* x;
   int x_layout;            // MM1_GEMM_ROW / _COL

@@ -116,7 +116,7 @@ struct Epilogue {
   const void *bias, *residual;
   void* out;
   __bf16* pre;
-  long ldr, ldp, ldo;      // bytes of a block's rows stay in 32 bits
+  long ldr, ldp, ldo;      // offsets in the EPILOGUE_ROWS of a wave's block stay in 32 bits
   int M, N, act;
   bool bias_f32, residual_f32, out_f32;
 };
@@ -190,6 +190,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, char* lds, int lane, l
   constexpr int LROWS = 16 / NB, STEPS = ROWS / LROWS;               // rows of an instruction
   static_assert(STEPS * LROWS == ROWS && 32 % ROWS == 0, "whole instructions");
   static_assert(!ACT || TI * TJ <= 8, "an activation takes the smaller tiles");
+  static_assert(32 * TI <= EPILOGUE_ROWS, "32-bit offsets");
   __asm__ volatile("" : "+v"(lane));       // made anew here: no address of the epilogue lives through the products
   const int l32 = lane & 31, h = lane >> 5, c8 = lane % (4 * NB), lr = lane / (4 * NB);
   auto swizzle = [](int row) { return NB == 2 ? row & 7 : (row >> 1) & 7; };

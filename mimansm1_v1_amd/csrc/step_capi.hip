@@ -28,7 +28,12 @@ bool embedding_sizes_ok(long tokens, int vocab, int dim) {
   return tokens * pieces <= (1L << 32) - 256 && (tokens + 7) / 8 * slabs < (1L << 24);
 }
 
-constexpr long kMaxEpilogueLd = 1L << 24;      // 32-bit offsets inside a block of 32 rows
+// A row stride that the epilogue takes: 32-bit byte offsets inside the rows of a wave's block, of
+// which it touches no more than M, up to 56 columns into a row.
+bool epilogue_ld_ok(long ld, bool f32, int M, int N) {
+  const long rows = M < mm1::EPILOGUE_ROWS ? M : mm1::EPILOGUE_ROWS;
+  return ld >= N && ld <= (1L << 24) && ((rows - 1) * ld + 64) * (f32 ? 4 : 2) <= (1L << 32);
+}
 
 bool linear_sizes_ok(int M, int N, int K) {
   return M >= 1 && N >= 1 && K >= 1 && M <= (1 << 28) && N <= (1 << 28) && K <= (1 << 28) &&
@@ -170,8 +175,8 @@ int mm1_linear(const void* x, int x_layout, long ldx, const void* w, int w_layou
   if (act < MM1_ACT_NONE || act > MM1_ACT_SILU || (xc && (act != MM1_ACT_NONE || pre))) return MM1_E_SHAPE;
   if (!linear_sizes_ok(M, N, K) || !operand_ok(x_layout, ldx, M, K) || !operand_ok(w_layout, ldw, N, K))
     return MM1_E_SHAPE;
-  if (ldo < N || ldo > kMaxEpilogueLd || (residual && (ldr < N || ldr > kMaxEpilogueLd)) ||
-      (pre && (ldp < N || ldp > kMaxEpilogueLd)))
+  if (!epilogue_ld_ok(ldo, out_f32, M, N) || (residual && !epilogue_ld_ok(ldr, residual_f32, M, N)) ||
+      (pre && !epilogue_ld_ok(ldp, false, M, N)))
     return MM1_E_SHAPE;
   if (!aligned(x, 16) || !aligned(w, 16) || !aligned(workspace, 16) || !element_aligned(out, out_f32) ||
       !element_aligned(bias, bias_f32) || !element_aligned(residual, residual_f32) || !aligned(pre, 2))
@@ -206,6 +211,9 @@ int mm1_linear_backward(const void* dy, int dy_f32, long ldy, const void* pre, l
   const int x_as = MM1_GEMM_COL, w_as = wc ? MM1_GEMM_ROW : MM1_GEMM_COL;    // as dW's and dX's products read them
   if ((dx && (ldw < (wc ? ceil8(N) : ceil8(K)) || !operand_ok(w_as, ldw, K, N))) ||
       (dw && (ldx < ceil8(K) || !operand_ok(x_as, ldx, K, M))))
+    return MM1_E_SHAPE;
+  if ((dx && !epilogue_ld_ok(K, dx_f32, M, K)) ||
+      (dw && !(wc ? epilogue_ld_ok(N, dw_f32, K, N) : epilogue_ld_ok(K, dw_f32, N, K))))
     return MM1_E_SHAPE;
   if (!element_aligned(dy, dy_f32) || !aligned(pre, 2) || !aligned(x, 16) || !aligned(w, 16) ||
       !element_aligned(dx, dx_f32) || !element_aligned(dw, dw_f32) || !element_aligned(dbias, dbias_f32) ||

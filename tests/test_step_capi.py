@@ -151,6 +151,26 @@ def test_linear_argument_errors(lib):
     assert product(lib, m=64, k=4096, ldx=4096, ldw=4096, ws=None) == -4
 
 
+def test_linear_refuses_strides_past_its_offsets(lib):
+    """A wave's 128 rows of the output or residual, or M where that is fewer, have
+    32-bit byte offsets: (rows - 1) ld + 64 elements at most 2^32 bytes.  What the
+    sizes let through is refused for its address, so that nothing is launched."""
+    far = ((1 << 30) - 64) // 127
+    for kw in (dict(m=1000, ldo=far + 1, out32=1), dict(m=128, ldo=1 << 24, out32=1),
+               dict(m=1000, res=FAKE, res32=1, ldr=far + 1), dict(m=64, ldo=(1 << 24) + 1),
+               dict(m=66, res=FAKE, res32=1, ldr=1 << 24)):
+        assert product(lib, **kw) == -2, kw
+    for kw in (dict(m=1000, ldo=far, out32=1), dict(m=64, ldo=1 << 24, out32=1), dict(m=1000, ldo=1 << 24),
+               dict(m=1000, res=FAKE, ldr=1 << 24), dict(m=1000, res=FAKE, res32=1, ldr=1 << 23),
+               dict(m=1000, act=4, pre=FAKE, ldp=1 << 24)):
+        assert product(lib, x=FAKE + 8, **kw) == -6, kw
+    wide = 8 * (far // 8 + 1)        # dX's and dW's rows are theirs whole
+    kw = dict(m=200, n=200, ldy=200, ldp=200, ldx=wide, ldw=wide, k=wide, db=None)
+    assert backward(lib, dx32=1, dw=None, **kw) == -2 and backward(lib, dx=None, dw32=1, **kw) == -2
+    assert backward(lib, dx32=1, dw=None, dy=FAKE + 1, **dict(kw, m=16)) == -6
+    assert backward(lib, dy=FAKE + 1, **kw) == -6
+
+
 def backward(lib, dy=FAKE, dy32=0, ldy=60, pre=FAKE, ldp=60, act=4, x=FAKE, ldx=40, w=FAKE, wl=0, ldw=40, dx=FAKE, dx32=0,
              dw=FAKE, dw32=0, db=FAKE, db32=1, ws=FAKE, nb=None, m=100, n=60, k=40):
     nb = lib.mm1_linear_backward_workspace_size(m, n, k, 1, 1, 1, 1) if nb is None else nb
