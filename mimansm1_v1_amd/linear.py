@@ -31,6 +31,8 @@ from .calls import F32, call, workspace
 
 DTYPE = torch.bfloat16
 ROW, COL = 0, 1                 # MM1_GEMM_ROW, MM1_GEMM_COL
+MAX_WIDTH = 4_000_000           # N and K whose rows the tiles' offsets reach, forward and backward
+MAX_ROWS = 1 << 28
 MAX_LD = 1 << 21                # longest row stride that the tiles' 32-bit offsets are sure to take
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}      # MM1_ACT_*
 
@@ -158,12 +160,20 @@ def _check(t, name, device, shape=None):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
+def _check_sizes(rows, n, k):
+    """What the library takes, before its 32-bit arguments."""
+    if n > MAX_WIDTH or k > MAX_WIDTH:
+        raise ValueError(f"N and K are at most {MAX_WIDTH:,}, got {n:,} and {k:,}")
+    if rows > MAX_ROWS:
+        raise ValueError(f"x has {rows:,} rows, at most {MAX_ROWS:,} are taken")
+
+
 def fused_linear(x, w, bias=None, activation="none", residual=None, out_dtype=None):
     """``act(x w^T + bias) + residual`` [..., N]: x [..., K] and w [N, K]
     (nn.Linear's layout, or the transposed view of a [K, N] matrix), bias [N]
     and residual [..., N] in fp32 or bf16; activation "none", "relu", "gelu",
     "gelu_tanh" or "silu".  The output is in ``out_dtype``, by default the
-    residual's, without one bf16.  N and K are at most 4,000,000."""
+    residual's, without one bf16.  N and K are at most 4,000,000, rows 2^28."""
     device = getattr(x, "device", None)
     _check(x, "x", device)
     _check(w, "w", device)
@@ -173,6 +183,8 @@ def fused_linear(x, w, bias=None, activation="none", residual=None, out_dtype=No
     x_shape, w_shape = x.shape, w.shape
     if len(w_shape) != 2 or not x_shape or x_shape[-1] != w_shape[1] or 0 in w_shape:
         raise ValueError(f"x has shape {tuple(x_shape)}, w {tuple(w_shape)}: [..., K] and [N, K] expected")
+    n, k = w_shape
+    _check_sizes(x.numel() // k, n, k)
     needs_grad = x.requires_grad or w.requires_grad
     if bias is not None:
         _check(bias, "bias", device, w_shape[:1])

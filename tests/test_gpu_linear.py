@@ -370,3 +370,12 @@ def test_refusals(hip_device):
     ]:
         with pytest.raises(error):
             bad()
+
+
+def test_sizes_past_the_documented_ones(hip_device):
+    """Refused before anything is allocated: N, K and rows, of views that take no memory."""
+    some = lambda rows, cols: torch.zeros(1, 1, device=hip_device, dtype=BF16).expand(rows, cols)
+    for x, w in ((some(2, 8), some(4_000_001, 8)), (some(2, 4_000_001), some(8, 4_000_001)),
+                 (some((1 << 28) + 1, 8), some(8, 8)), (some((1 << 32) + 5, 8), some(8, 8))):
+        with pytest.raises(ValueError, match="at most"):
+            linear.fused_linear(x, w)

@@ -210,3 +210,16 @@ def test_linear_refuses_cpu_tensors():
         linear.fused_linear(torch.zeros(2, 8), torch.zeros(4, 8))
     with pytest.raises(TypeError):
         linear.fused_linear([1.0], torch.zeros(4, 8))
+
+
+def test_linear_refuses_sizes_past_the_librarys():
+    """The documented widths, which an operand's own checks let past for one of the
+    two, and row counts before they wrap in a 32-bit argument."""
+    from mimansm1_v1_amd import linear
+    check = linear._check_sizes
+    check(1 << 28, 4_000_000, 1)
+    check(0, 1, 4_000_000)
+    for rows, n, k in ((1, 4_000_001, 8), (1, 8, 4_000_001), (1, (1 << 32) + 8, 8), ((1 << 28) + 1, 8, 8),
+                       ((1 << 32) + 5, 8, 8)):
+        with pytest.raises(ValueError, match="at most"):
+            check(rows, n, k)
