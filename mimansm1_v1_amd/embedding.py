@@ -23,6 +23,14 @@ import torch.nn as nn
 from . import _lib
 from .calls import F32, call, workspace, written
 
+MAX_VOCAB, MAX_DIM = 1 << 30, (1 << 31) - 1     # what the library's 32-bit arguments hold
+
+
+def _check_sizes(vocab, dim):
+    if not 1 <= vocab <= MAX_VOCAB or not 1 <= dim <= MAX_DIM:
+        raise ValueError(f"a matrix of {vocab:,} rows and {dim:,} columns: 1 to {MAX_VOCAB:,} rows are taken, of 1 to "
+                         f"{MAX_DIM:,} columns")
+
 
 def _check_ids(ids):
     if not isinstance(ids, torch.Tensor):
@@ -43,8 +51,7 @@ def _check_rows(t, name, device, shape=None):
         raise TypeError(f"{name} must be fp32 or bf16, got {t.dtype}")
     if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape) if shape else '[vocab, dim]'}")
-    if t.shape[1] < 1 or t.shape[0] < 1:
-        raise ValueError(f"{name} has no rows or no columns")
+    _check_sizes(*t.shape)
     if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         raise ValueError(f"{name} must have rows of consecutive values that do not overlap, got strides {t.stride()}")
 
@@ -102,9 +109,8 @@ def embedding_grad(ids, grad_out, vocab, scale=1.0, padding_idx=None, dtype=torc
         raise TypeError(f"grad_out must be fp32 or bf16, got {grad_out.dtype}")
     if grad_out.dim() < 1 or grad_out.shape[:-1] != ids.shape or grad_out.shape[-1] < 1:
         raise ValueError(f"grad_out has shape {tuple(grad_out.shape)}, expected {tuple(ids.shape)} and a width")
-    if vocab < 1:
-        raise ValueError(f"vocab must be positive, got {vocab}")
     dim = grad_out.shape[-1]
+    _check_sizes(vocab, dim)
     padding = _padding(padding_idx, vocab)
     if out is None:
         if accumulate:

@@ -267,3 +267,12 @@ def test_refusals(hip_device):
     ]:
         with pytest.raises(error):
             bad()
+
+
+def test_sizes_past_the_librarys(hip_device):
+    """Refused before anything is allocated."""
+    ids, dy = torch.zeros(4, dtype=torch.int64, device=hip_device), torch.zeros(4, 1, device=hip_device)
+    wide = torch.zeros(1, device=hip_device, dtype=BF16).expand((1 << 32) + 10, 1)
+    for bad in (lambda: embedding.embedding_grad(ids, dy, (1 << 32) + 10), lambda: embedding.embed(ids, wide)):
+        with pytest.raises(ValueError, match="rows are taken"):
+            bad()

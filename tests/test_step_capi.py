@@ -223,3 +223,13 @@ def test_linear_refuses_sizes_past_the_librarys():
                        ((1 << 32) + 5, 8, 8)):
         with pytest.raises(ValueError, match="at most"):
             check(rows, n, k)
+
+
+def test_embedding_refuses_sizes_past_the_librarys():
+    """Rows and columns before they wrap in a 32-bit argument."""
+    check = embedding._check_sizes
+    check(1 << 30, 1)
+    check(1, (1 << 31) - 1)
+    for vocab, dim in ((0, 8), (8, 0), ((1 << 30) + 1, 8), ((1 << 32) + 10, 8), (8, (1 << 32) + 8)):
+        with pytest.raises(ValueError, match="rows are taken"):
+            check(vocab, dim)
