@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -26,6 +27,15 @@ def call(name: str, device, *args) -> None:
             rc = fn(*args, stream)
     if rc:
         _lib.check(rc, name)
+
+
+def refuse_tangents(name: str, tensors) -> None:
+    """Raises where a tensor (None is none) carries a forward-mode tangent, as an
+    autograd.Function without a jvp does: a call that goes to the kernels past
+    autograd would drop it."""
+    if forward_ad._current_level >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def workspace(nbytes: int, device):

@@ -4,7 +4,8 @@ whose tied output head (``lm_head.py``) reads the same matrix.  The reference
 uses torch's ``nn.Embedding`` there (CODE/mimans/model/model.py:53-127).
 
 * ``embed(ids, weight, scale, padding_idx, out_dtype)``: rows of ``weight``
-  times ``scale``, differentiable in ``weight`` (any number of times);
+  times ``scale``, differentiable in ``weight`` (any number of times,
+  in reverse; forward-mode tangents are refused);
 * ``embedding_grad(ids, grad_out, vocab, ...)``: the matrix's gradient, new or
   added to one that is there (the tied head's);
 * ``Embedding``: an ``nn.Embedding`` whose lookup runs here, to be handed to
@@ -21,7 +22,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .calls import F32, call, workspace, written
+from .calls import F32, call, refuse_tangents, workspace, written
 
 MAX_VOCAB, MAX_DIM = 1 << 30, (1 << 31) - 1     # what the library's 32-bit arguments hold
 
@@ -100,6 +101,7 @@ def embedding_grad(ids, grad_out, vocab, scale=1.0, padding_idx=None, dtype=torc
     stride of its own) or to a new tensor of ``dtype``; with ``accumulate`` the
     sums are added to ``out``, whose other rows are left as they are.  Leaves
     no autograd graph."""
+    refuse_tangents("embedding_grad", (grad_out, out))
     _check_ids(ids)
     if not isinstance(grad_out, torch.Tensor):
         raise TypeError("grad_out must be a torch.Tensor")
@@ -169,6 +171,7 @@ def embed(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
     """``scale * weight[ids]`` [*ids.shape, dim] in ``out_dtype`` (default: the
     weight's), from a [vocab, dim] matrix in fp32 or bf16.  ``padding_idx``:
     the row that takes no gradient (it is looked up like any other)."""
+    refuse_tangents("embed", (weight,))
     _check_ids(ids)
     _check_rows(weight, "weight", ids.device)
     out_dtype = weight.dtype if out_dtype is None else out_dtype

@@ -23,7 +23,7 @@ from array import array
 import torch
 
 from . import _lib
-from .calls import F32, call, workspace, written
+from .calls import F32, call, refuse_tangents, workspace, written
 
 EPS = 1e-6
 NORMS = {2.0: 0, math.inf: 1}        # MM1_NORM_2, MM1_NORM_MAX
@@ -175,6 +175,7 @@ def _any_needs_grad(tensors):
 
 
 def _unrecorded(tensors):
+    refuse_tangents("the norm", tensors)
     if torch.is_grad_enabled() and _any_needs_grad(tensors):
         raise RuntimeError("the norm and the clipped gradients leave no autograd graph: call under torch.no_grad()")
 
@@ -211,6 +212,7 @@ def clip_grads(tensors, max_norm, norm_type=2.0, out=None):
         return [], torch.tensor(0.0)
     _unrecorded(tensors)
     to = tensors if same else out if out is not None else [torch.empty_like(t) for t in tensors]
+    refuse_tangents("the norm", to)
     if out is not None and _any_needs_grad(to):
         raise ValueError("out must not require a gradient: it is written in place")
     table = _Table(tensors, to)
@@ -229,6 +231,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     raises before anything is scaled."""
     grads = [p.grad for p in _list(parameters) if p.grad is not None]
     code, max_norm = _norm_code(norm_type), _max_norm(max_norm)
+    refuse_tangents("the norm", grads)
     if not grads:
         return torch.tensor(0.0)
     table = _Table(grads, grads)

@@ -5,7 +5,8 @@ torch product and an addition (CODE/mimans/model/attention_tilelang.py:518,
 swiglu_tilelang.py:284-286, block.py:81-92).
 
 * ``fused_linear(x, w, bias, activation, residual, out_dtype)``:
-  ``act(x w^T + bias) + residual``, differentiable once in every tensor;
+  ``act(x w^T + bias) + residual``, differentiable once in every tensor
+  (in reverse; forward-mode tangents are refused);
 * ``Linear``: an ``nn.Linear`` with an activation whose forward takes a residual.
 
 ``Attention`` and ``SwiGLU`` call it for their last product when they are given
@@ -27,7 +28,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .calls import F32, call, workspace
+from .calls import F32, call, refuse_tangents, workspace
 
 DTYPE = torch.bfloat16
 ROW, COL = 0, 1                 # MM1_GEMM_ROW, MM1_GEMM_COL
@@ -174,6 +175,7 @@ def fused_linear(x, w, bias=None, activation="none", residual=None, out_dtype=No
     and residual [..., N] in fp32 or bf16; activation "none", "relu", "gelu",
     "gelu_tanh" or "silu".  The output is in ``out_dtype``, by default the
     residual's, without one bf16.  N and K are at most 4,000,000, rows 2^28."""
+    refuse_tangents("fused_linear", (x, w, bias, residual))
     device = getattr(x, "device", None)
     _check(x, "x", device)
     _check(w, "w", device)

@@ -32,7 +32,7 @@ import torch.nn.functional as F
 from . import _lib
 from . import gemm
 from . import tuned
-from .calls import F32
+from .calls import F32, refuse_tangents
 from .harness import Report, compare, needs_gpu, time_cuda
 from .harness import main as harness_main
 from .linear import fused_linear
@@ -316,6 +316,7 @@ def fused_swiglu(x, w_gate, w_up, w_down, residual=None, out_dtype=None):
     bf16) added to it in the down projection's epilogue, in ``out_dtype`` (default
     the residual's) with one rounding."""
     if residual is not None:
+        refuse_tangents("fused_swiglu", (x, w_gate, w_up, w_down, residual))
         act = FusedGateUp.apply(x, w_gate, w_up) if torch.is_grad_enabled() else \
             get_kernel("train", x.shape[0], x.shape[1], w_gate.shape[1]).act_only(x, w_gate, w_up)
         return fused_linear(act, w_down.t(), residual=residual, out_dtype=out_dtype)

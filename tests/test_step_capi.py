@@ -233,3 +233,37 @@ def test_embedding_refuses_sizes_past_the_librarys():
     for vocab, dim in ((0, 8), (8, 0), ((1 << 30) + 1, 8), ((1 << 32) + 10, 8), (8, (1 << 32) + 8)):
         with pytest.raises(ValueError, match="rows are taken"):
             check(vocab, dim)
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_tangents_are_refused(grad_mode):
+    """No call drops a tangent: each raises before it looks at devices."""
+    from torch.autograd import forward_ad
+
+    from mimansm1_v1_amd import linear, swiglu
+    ids = torch.zeros(4, dtype=torch.int64)
+    square = lambda: torch.zeros(4, 4)
+    with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+        dual = forward_ad.make_dual(square(), torch.ones(4, 4))
+        row = forward_ad.make_dual(torch.zeros(4), torch.ones(4))
+        calls = [lambda: linear.fused_linear(dual, square()), lambda: linear.fused_linear(square(), dual),
+                 lambda: linear.fused_linear(square(), square(), row),
+                 lambda: linear.fused_linear(square(), square(), residual=dual),
+                 lambda: linear.Linear(4, 4)(dual), lambda: embedding.embed(ids, dual),
+                 lambda: embedding.embedding_grad(ids, dual, 4),
+                 lambda: embedding.embedding_grad(ids, square(), 4, out=dual),
+                 lambda: grad_clip.grad_norm([square(), dual]), lambda: grad_clip.clip_grads([dual], 1.0),
+                 lambda: grad_clip.clip_grads([square()], 1.0, out=[dual])]
+        calls += [lambda i=i: swiglu.fused_swiglu(*(dual if j == i else square() for j in range(4)), residual=square())
+                  for i in range(4)]
+        calls.append(lambda: swiglu.fused_swiglu(*(square() for _ in range(4)), residual=dual))
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        parameter = torch.nn.Parameter(square())
+        parameter.grad = dual
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            grad_clip.clip_grad_norm_([parameter], 1.0)
+        # beside duals that are not an input's, calls go on as ever
+        with pytest.raises(ValueError, match="CUDA"):
+            linear.fused_linear(square(), square())
