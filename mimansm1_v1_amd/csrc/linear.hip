@@ -77,7 +77,7 @@ __device__ __forceinline__ float act1(float z) {
 
 template <int ACT>
 __device__ __forceinline__ float slope1(float z) {
-  if constexpr (ACT == RELU) return z > 0.f ? 1.f : 0.f;
+  if constexpr (ACT == RELU) return z <= 0.f ? 0.f : 1.f;             // a NaN hands dY on
   if constexpr (ACT == SILU) {
     const float s = sigmoid(z);
     return fabsf(z) > 80.f ? (z > 0.f ? 1.f : 0.f) : s * fmaf(z, 1.f - s, 1.f);

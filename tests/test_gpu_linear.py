@@ -379,3 +379,32 @@ def test_sizes_past_the_documented_ones(hip_device):
                  (some((1 << 28) + 1, 8), some(8, 8)), (some((1 << 32) + 5, 8), some(8, 8))):
         with pytest.raises(ValueError, match="at most"):
             linear.fused_linear(x, w)
+
+
+def infinite_and_missing(rows, dev):
+    """x and w whose z = x w^T has +inf, -inf and NaN in its last three rows, ones before."""
+    x = torch.zeros(rows, 1280, dtype=BF16, device=dev)
+    x[:, 0] = 1
+    x[rows - 3:, 0] = torch.tensor([float("inf"), -float("inf"), float("nan")], device=dev)
+    w = torch.zeros(1280, 1280, dtype=BF16, device=dev)
+    w[:, 0] = 1
+    return x, w
+
+
+@pytest.mark.parametrize("rows", [3, 40, 2100])
+@pytest.mark.parametrize("act", ACTS)
+def test_slopes_of_infinite_and_missing_values(hip_device, act, rows):
+    """dx = dy slope(z): 1 at +inf, 0 at -inf; at a NaN relu hands dy on, the others'
+    slope is NaN.  The rows around them stay finite."""
+    nan = float("nan")
+    x, w = infinite_and_missing(rows, hip_device)
+    x.requires_grad_(True)
+    y = linear.fused_linear(x, w, activation=act, out_dtype=FP32)
+    dy = torch.zeros_like(y)
+    dy[:, 5] = 2                                     # dx is dz w: dz's one column, in dx's first
+    (dx,) = torch.autograd.grad(y, x, dy)
+    wants = (2.0, 2.0 if act == "none" else 0.0, 2.0 if act in ("none", "relu") else nan)
+    got = dx[rows - 3:, 0].float().tolist()
+    for g, want in zip(got, wants):
+        assert g != g if want != want else abs(g - want) <= 1e-30, (act, got)
+    assert bool(torch.isfinite(dx[:rows - 3]).all())
