@@ -40,7 +40,8 @@ __device__ __forceinline__ float exp_fast(float x) { return exp2_fast(x * 1.4426
 // The normal distribution's upper tail Q(a) for a >= 0 and its density
 // exp(-a^2 / 2) (times sqrt(2 pi)): Q = density * t P(t), t = 1 / (1 + 0.265 a), P the
 // polynomial of least relative error over a in [0, 13.5] (6.3e-7; fitted to
-// erfcx by weighted least squares), beyond which Q is below 2^-126.
+// erfcx by weighted least squares), beyond which Q is below 2^-126.  The density is 0
+// from 15 on, so that arguments clamped to 16 give Q = 0.
 __device__ __forceinline__ float upper_tail(float a, float& density) {
   const float t = recip(fmaf(0.265f, a, 1.f));
   float p = -0.0677873029f;
@@ -68,7 +69,7 @@ __device__ __forceinline__ float act1(float z) {
     return u < -80.f ? 0.f : z * sigmoid(u);
   }
   if constexpr (ACT == GELU) {
-    const float a = fminf(fabsf(z), 13.f);
+    const float a = fminf(fabsf(z), 16.f);
     float d;
     return (z < 0.f ? 0.f : z) - a * upper_tail(a, d);       // max(z, 0) - |z| Q(|z|)
   }
@@ -88,7 +89,7 @@ __device__ __forceinline__ float slope1(float z) {
     return fabsf(u) > 80.f ? (z > 0.f ? 1.f : 0.f) : s * fmaf(z * du, 1.f - s, 1.f);
   }
   if constexpr (ACT == GELU) {
-    const float a = fminf(fabsf(z), 13.f);
+    const float a = fminf(fabsf(z), 16.f);
     float d;
     const float q = upper_tail(a, d), t = fmaf(a, -0.3989422804f * d, q);      // Q(a) - a density(a)
     return z < 0.f ? t : z != z ? z : 1.f - t;

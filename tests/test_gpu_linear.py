@@ -408,3 +408,19 @@ def test_slopes_of_infinite_and_missing_values(hip_device, act, rows):
     for g, want in zip(got, wants):
         assert g != g if want != want else abs(g - want) <= 1e-30, (act, got)
     assert bool(torch.isfinite(dx[:rows - 3]).all())
+
+
+@pytest.mark.parametrize("rows", [3, 40, 2100])
+@pytest.mark.parametrize("act", ACTS)
+def test_infinite_and_missing_values(hip_device, act, rows):
+    """+inf stays, -inf becomes the activations' limit 0, a NaN stays one; the rows
+    around them stay finite.  gelu's tail vanishes before -20 too."""
+    x, w = infinite_and_missing(rows, hip_device)
+    inf, nan = float("inf"), float("nan")
+    y = linear.fused_linear(x, w, activation=act, out_dtype=FP32)
+    for row, want in zip(y[rows - 3:], (inf, -inf if act == "none" else 0.0, nan)):
+        assert bool((row.isnan() if want != want else row == want).all()), (act, want, row[:4])
+    assert bool(torch.isfinite(y[:rows - 3]).all())
+    if act == "gelu":
+        x[rows - 3:, 0] = torch.tensor([-20, -1e4, -3e38], device=hip_device)
+        assert not linear.fused_linear(x, w, activation=act, out_dtype=FP32)[rows - 3:].any()
