@@ -38,7 +38,8 @@ size_t mm1_embedding_grad_workspace_size(long tokens, int vocab, int dim);
  * without tokens are cleared.  With accumulate the sums are added to grad, in
  * fp32 with one rounding, and rows without tokens are left as they are.
  * padding_idx: the row that takes no gradient, -1 for none.  ld_d_out may be 0
- * (one gradient row for every token). */
+ * (one gradient row for every token).  grad shares no memory with ids or d_out:
+ * it is cleared and written while they are read. */
 int mm1_embedding_grad(const void* ids, int ids_wide, const void* d_out, int d_out_f32, long ld_d_out, void* grad,
                        int grad_f32, long ldg, float scale, long padding_idx, int accumulate, void* workspace,
                        size_t workspace_bytes, long tokens, int vocab, int dim, void* stream);

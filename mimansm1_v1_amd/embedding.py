@@ -61,6 +61,29 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _extent(t):
+    """The bytes [first, last) that a tensor's values lie in (with what lies between them)."""
+    last = sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride())) + 1
+    return t.data_ptr(), t.data_ptr() + last * t.element_size()
+
+
+def _shares(out, t):
+    """Whether `out`, rows of values, may share memory with `t`: their extents meet
+    and they are not different columns of rows equally far apart."""
+    if not t.numel():
+        return False
+    (a0, a1), (b0, b1) = _extent(out), _extent(t)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    pitch, width = out.stride(0) * out.element_size(), out.shape[1] * out.element_size()
+    steps = [(n, s) for n, s in zip(t.shape, t.stride()) if n > 1]
+    cols = steps.pop()[0] if steps and steps[-1][1] == 1 else 1
+    if pitch == 0 or any(s * t.element_size() % pitch for _, s in steps):
+        return True
+    at, wide = (b0 - a0) % pitch, cols * t.element_size()      # t's columns seen from out's first
+    return at < width or at + wide > pitch
+
+
 def _padding(padding_idx, vocab):
     """-1 for none; a negative index counts from the end, as in nn.Embedding."""
     if padding_idx is None:
@@ -99,8 +122,8 @@ def embedding_grad(ids, grad_out, vocab, scale=1.0, padding_idx=None, dtype=torc
     """[vocab, dim]: row v is ``scale`` times the sum of ``grad_out`` [..., dim]
     over the tokens whose id is v.  Written to ``out`` (its own dtype; a row
     stride of its own) or to a new tensor of ``dtype``; with ``accumulate`` the
-    sums are added to ``out``, whose other rows are left as they are.  Leaves
-    no autograd graph."""
+    sums are added to ``out``, whose other rows are left as they are.  ``out``
+    shares no memory with the inputs.  Leaves no autograd graph."""
     refuse_tangents("embedding_grad", (grad_out, out))
     _check_ids(ids)
     if not isinstance(grad_out, torch.Tensor):
@@ -124,6 +147,8 @@ def embedding_grad(ids, grad_out, vocab, scale=1.0, padding_idx=None, dtype=torc
     _check_rows(out, "out", ids.device, (vocab, dim))
     if out.requires_grad:
         raise ValueError("out must not require a gradient: it is written in place")
+    if _shares(out, grad_out) or _shares(out, ids):
+        raise ValueError("out must not share memory with grad_out or ids: it is written while they are read")
     _gradient(ids, grad_out.detach(), scale, padding, out, accumulate)
     written(out)
     return out

@@ -276,3 +276,25 @@ def test_sizes_past_the_librarys(hip_device):
     for bad in (lambda: embedding.embedding_grad(ids, dy, (1 << 32) + 10), lambda: embedding.embed(ids, wide)):
         with pytest.raises(ValueError, match="rows are taken"):
             bad()
+
+
+def test_gradient_into_its_inputs_memory_is_refused(hip_device):
+    """Clearing or writing the matrix would change what the sums still read; other
+    columns of the same rows are memory of their own."""
+    gen = torch.Generator(hip_device).manual_seed(12)
+    store = torch.randn(300, 96, device=hip_device, generator=gen)
+    ids = make_ids("random", 300, 200, gen, hip_device)
+    before = store.clone()
+    for accumulate in (False, True):
+        for out, dy in ((store[:200, :40], store[:, :40]), (store[:200, :40], store[:, 39:79]),
+                        (store[100:, :40], store.view(-1)[:12000].view(300, 40)), (store[:200, :40], store[7, :40].expand(300, 40))):
+            with pytest.raises(ValueError, match="share memory"):
+                embedding.embedding_grad(ids, dy, 200, out=out, accumulate=accumulate)
+        inside = store.view(torch.int64)[:200, 0]
+        with pytest.raises(ValueError, match="share memory"):
+            embedding.embedding_grad(inside, store[:200, 40:80], 200, out=store[:200, :40], accumulate=accumulate)
+    assert torch.equal(store, before)
+    store.view(torch.int64)[:, 47] = ids
+    embedding.embedding_grad(store.view(torch.int64)[:, 47], store[:, 40:80], 200, out=store[:200, :40])
+    check_grad(store[:200, :40], ids, before[:, 40:80], 1.0)
+    assert torch.equal(store[:, 40:94], before[:, 40:94]) and torch.equal(store[200:, :94], before[200:, :94])

@@ -267,3 +267,21 @@ def test_forward_mode_tangents_are_refused(grad_mode):
         # beside duals that are not an input's, calls go on as ever
         with pytest.raises(ValueError, match="CUDA"):
             linear.fused_linear(square(), square())
+
+
+def test_memory_shared_with_the_gradients_output():
+    """Shared values are found whatever the views; neighbours, other columns of the
+    same rows and other rows are let through."""
+    store = torch.zeros(40, 16)
+    out = store[:10, :8]
+    for t in (out, store[:4, :8], store[9:12, :8], store[2:6, 7:9], store[::3, 4:10], store.view(-1)[:80].view(10, 8),
+              store[:10, :8].t(), store[0, 3], store[:5, 12:].as_strided((5, 8), (16, 1)), store[3].expand(4, 16),
+              store.view(20, 2, 16)[:, :, :2], store.view(torch.int32)[5], store.view(torch.int64)[:, 3:5],
+              store.view(-1)[-632:].view(79, 8), store[:, 7], store.view(torch.int64)[:, 0]):
+        assert embedding._shares(out, t), (t.shape, t.stride())
+    for t in (store[10:20, :8], store[:10, 8:], store[::2, 9:12], torch.zeros(10, 8), store[:0, :8], store[12, 8:].expand(4, 8),
+              store.view(torch.int64)[:, 4:], store.view(2, 20, 16)[:, ::5, 10:], store[0, 8:], store[20:30, :8],
+              store[:, 9], store.view(torch.int64)[:, 7], store[2, 12], store[:0]):
+        assert not embedding._shares(out, t), (t.shape, t.stride())
+    assert embedding._shares(store, store[3:4, 2:3]) and not embedding._shares(store[:10], store[10:])
+    assert embedding._shares(store[3:4], store[3]) and not embedding._shares(store[3:4], store[4])
