@@ -313,9 +313,11 @@ class _FusedSwiGLUNoGrad(torch.autograd.Function):
 
 def fused_swiglu(x, w_gate, w_up, w_down, residual=None, out_dtype=None):
     """(silu(x w_gate) * (x w_up)) w_down; with ``residual`` [T, d_model] (fp32 or
-    bf16) added to it in the down projection's epilogue, in ``out_dtype`` (default
-    the residual's) with one rounding."""
-    if residual is not None:
+    bf16) added to it in the down projection's epilogue.  The output is in
+    ``out_dtype`` (default the residual's, without one bf16) with one rounding."""
+    if out_dtype is not None and out_dtype not in F32:
+        raise TypeError(f"out_dtype must be fp32 or bf16, got {out_dtype}")
+    if residual is not None or out_dtype not in (None, DTYPE):
         refuse_tangents("fused_swiglu", (x, w_gate, w_up, w_down, residual))
         act = FusedGateUp.apply(x, w_gate, w_up) if torch.is_grad_enabled() else \
             get_kernel("train", x.shape[0], x.shape[1], w_gate.shape[1]).act_only(x, w_gate, w_up)

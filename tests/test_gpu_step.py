@@ -160,3 +160,29 @@ def test_greedy_single_tokens_without_gradients(hip_device):
             one = mm.fused_linear(x[i], w, residual=x[i], out_dtype=torch.float32)
             size = x[i].float().abs() @ w.float().abs().t() + x[i].float().abs()
             assert one.shape == (D,) and bool(((one - full[i]).abs() <= 2 * (D + 2) * 2.0 ** -24 * size).all())
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_swiglu_output_type_without_a_residual(hip_device, train):
+    """fused_swiglu(..., out_dtype): fp32 outputs are the same sums before their one
+    rounding, so that rounding them gives the bf16 ones but for the sums' order;
+    gradients flow through both."""
+    gen = torch.Generator(hip_device).manual_seed(5)
+    randn = lambda *s: torch.randn(*s, device=hip_device, generator=gen).to(torch.bfloat16)
+    x, ws = randn(70, D), [randn(D, 384) / 16, randn(D, 384) / 16, randn(384, D) / 16]
+    leaves = [t.requires_grad_(train) for t in (x, *ws)]
+    wide, half = S.fused_swiglu(*leaves, out_dtype=torch.float32), S.fused_swiglu(*leaves)
+    assert wide.dtype == torch.float32 and half.dtype == torch.bfloat16
+    assert torch.equal(S.fused_swiglu(*leaves, out_dtype=torch.bfloat16), half)
+    with torch.no_grad():
+        act = S.fused_swiglu(x, ws[0], ws[1], torch.eye(384, device=hip_device, dtype=torch.bfloat16))
+    size = act.double().abs() @ ws[2].detach().double().abs()
+    want = act.double() @ ws[2].detach().double()
+    bound = 384 * 2.0 ** -24 * size                  # of 384 fp32 additions
+    assert bool(((wide.detach().double() - want).abs() <= 1.01 * bound + 2.0 ** -24 * want.abs()).all())
+    assert bool(((half.detach().double() - want).abs() <= 1.01 * bound + 2.0 ** -8 * (want.abs() + bound)).all())
+    if train:
+        dy = randn(70, D)
+        for a, b in zip(torch.autograd.grad(wide, leaves, dy.float()), torch.autograd.grad(half, leaves, dy)):
+            # the same bf16 products, summed in other orders and rounded to bf16 at each of two steps
+            assert (a.double() - b.double()).norm() <= 4 * 2.0 ** -8 * b.double().norm()

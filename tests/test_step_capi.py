@@ -285,3 +285,12 @@ def test_memory_shared_with_the_gradients_output():
         assert not embedding._shares(out, t), (t.shape, t.stride())
     assert embedding._shares(store, store[3:4, 2:3]) and not embedding._shares(store[:10], store[10:])
     assert embedding._shares(store[3:4], store[3]) and not embedding._shares(store[3:4], store[4])
+
+
+def test_swiglu_refuses_other_output_types():
+    from mimansm1_v1_amd import swiglu
+    ts = [torch.zeros(128, 128, dtype=torch.bfloat16)] * 4
+    for residual in (None, ts[0]):
+        for bad in (torch.float16, torch.float64, "fp32"):
+            with pytest.raises(TypeError, match="out_dtype"):
+                swiglu.fused_swiglu(*ts, residual, bad)
