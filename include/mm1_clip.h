@@ -41,7 +41,8 @@ int mm1_grad_norm(int count, const void* const* in, const long* rows, const long
  * to its type, and the norm before clipping; a NaN norm makes every value NaN.
  * out NULL: in place (then nothing is written where nothing is clipped); else
  * its tensors have the types, rows and cols of in, runs ld_out[i] apart, and
- * no two tensors that are written may share memory.  norm_known: *norm holds
+ * no two tensors that are written may share memory, and out[i] lies at in[i] or in
+ * no tensor of in (nor in norm).  norm_known: *norm holds
  * the norm already and is read, not computed.  max_norm >= 0, eps >= 0. */
 int mm1_grad_clip(int count, const void* const* in, void* const* out, const long* rows, const long* cols,
                   const long* ld, const long* ld_out, const unsigned char* f32, int norm_type, float max_norm,

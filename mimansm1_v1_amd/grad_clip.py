@@ -122,11 +122,14 @@ class _Table:
     def _refuse_shared(tensors, out):
         """An output may be its own gradient and nobody else's: another's would be
         overwritten before or after it is read, as the workgroups happen to run."""
-        read = {t.data_ptr(): i for i, t in enumerate(tensors) if t.numel()}
+        read = {}                         # the gradients at an address: the same one may be given twice
+        for i, t in enumerate(tensors):
+            if t.numel():
+                read.setdefault(t.data_ptr(), []).append(i)
         for i, o in enumerate(out):
-            j = read.get(o.data_ptr()) if o.numel() else None
-            if j is not None and (j != i or tensors[i].stride() != o.stride()):
-                raise ValueError(f"out[{i}] lies in the memory of gradient {j}")
+            for j in read.get(o.data_ptr(), ()) if o.numel() else ():
+                if j != i or tensors[i].stride() != o.stride():
+                    raise ValueError(f"out[{i}] lies in the memory of gradient {j}")
 
     def _strided(self, tensors, out):
         empty = ([], 0, 0, 0)

@@ -242,3 +242,18 @@ def test_refusals(hip_device):
         with pytest.raises(error):
             bad()
     assert grad_clip.grad_norm([]).item() == 0 and grad_clip.clip_grads([], 1.0)[0] == []
+
+
+def test_a_gradient_given_twice(hip_device):
+    """Its values count twice; its results are two new tensors, or two given ones, but
+    never its own memory, which the other reading would see half clipped."""
+    t, new = torch.randn(300, 70, device=hip_device), [torch.empty(300, 70, device=hip_device) for _ in range(2)]
+    before = t.clone()
+    for out in ([new[0], t], [t, new[0]]):
+        with pytest.raises(ValueError, match="memory of gradient"):
+            grad_clip.clip_grads([t, t], 0.5, out=out)
+    for out in (None, new):
+        clipped, norm = grad_clip.clip_grads([t, t], 0.5, out=out)
+        assert abs(norm.item() - exact_norm([t, t], 2.0)) <= 1.01 * U * exact_norm([t, t], 2.0)
+        check_clipped(clipped, [before, before], exact_norm([t, t], 2.0), 0.5)
+    assert torch.equal(t, before)

@@ -294,3 +294,17 @@ def test_swiglu_refuses_other_output_types():
         for bad in (torch.float16, torch.float64, "fp32"):
             with pytest.raises(TypeError, match="out_dtype"):
                 swiglu.fused_swiglu(*ts, residual, bad)
+
+
+def test_clip_outputs_in_a_gradient_given_twice():
+    """A gradient that is given twice is read twice, so an output may lie in neither's
+    memory, whichever of the two it belongs to."""
+    a, b, c = (torch.zeros(6, 4) for _ in range(3))
+    refuse = grad_clip._Table._refuse_shared
+    for out in ([a, b], [b, a], [a, a]):
+        with pytest.raises(ValueError, match="memory of gradient"):
+            refuse([a, a], out)
+    with pytest.raises(ValueError, match="memory of gradient 0"):
+        refuse([a, b, a], [c, b, a])
+    refuse([a, b], [a, c])
+    refuse([a, a, b], [torch.zeros(6, 4), c, b])
