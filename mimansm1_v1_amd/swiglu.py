@@ -388,7 +388,8 @@ class SwiGLU(nn.Module):
         if residual is not None:
             if residual.shape != x.shape:
                 raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {tuple(x.shape)}")
-            if runs[backend] == self._run_hip and residual.dtype in F32:
+            if runs[backend] == self._run_hip and residual.dtype in F32 and torch.promote_types(residual.dtype,
+                                                                                                x.dtype) in F32:
                 return self._run_hip(x.reshape(-1, self.cfg.d_model), x.dtype,
                                      residual.reshape(-1, self.cfg.d_model)).reshape(x.shape)
             return residual + self.forward(x, backend)

@@ -186,3 +186,21 @@ def test_swiglu_output_type_without_a_residual(hip_device, train):
         for a, b in zip(torch.autograd.grad(wide, leaves, dy.float()), torch.autograd.grad(half, leaves, dy)):
             # the same bf16 products, summed in other orders and rounded to bf16 at each of two steps
             assert (a.double() - b.double()).norm() <= 4 * 2.0 ** -8 * b.double().norm()
+
+
+@pytest.mark.parametrize("x_type", [torch.float16, torch.float64])
+def test_residual_beside_inputs_of_other_types(hip_device, x_type):
+    """Inputs that the sublayer takes without a residual it takes with one, in the
+    addition's type."""
+    torch.manual_seed(0)
+    ffn = S.SwiGLU(S.FFNConfig(D, 384)).to(hip_device)
+    x = torch.randn(2, SEQ, D, device=hip_device).to(x_type)
+    for r_type in (torch.float32, torch.bfloat16):
+        r = torch.randn(2, SEQ, D, device=hip_device).to(r_type)
+        with torch.no_grad():
+            y, got = ffn(x), ffn(x, residual=r)
+        want = r + y
+        assert got.dtype == want.dtype
+        # y is rounded to bf16 before the addition there, and the sums' order differs
+        bound = 2.0 ** -8 * y.double().abs() + 2.0 ** -12 * y.double().abs().max() + 2.0 ** -24 * want.double().abs()
+        assert bool(((got.double() - want.double()).abs() <= bound).all())
