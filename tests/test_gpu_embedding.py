@@ -298,3 +298,87 @@ def test_gradient_into_its_inputs_memory_is_refused(hip_device):
     embedding.embedding_grad(store.view(torch.int64)[:, 47], store[:, 40:80], 200, out=store[:200, :40])
     check_grad(store[:200, :40], ids, before[:, 40:80], 1.0)
     assert torch.equal(store[:, 40:94], before[:, 40:94]) and torch.equal(store[200:, :94], before[200:, :94])
+
+
+# The sort takes several workgroups from 16,385 tokens on, units of 32 tokens there and of 48 from
+# 32,769 on, and passes' counts in global memory from 524,289 on (65 tiles of 8192).
+@pytest.mark.parametrize("kind", ["random", "same", "few", "outside", "padded", "sorted"])
+@pytest.mark.parametrize("n", [16384, 16385, 32768, 32769, 50021])
+def test_gradient_where_the_sort_changes(hip_device, kind, n):
+    gen = torch.Generator(hip_device).manual_seed(n)
+    ids = make_ids(kind, n, 1009, gen, hip_device)
+    dy = torch.randn(n, 40, device=hip_device, generator=gen).to(BF16)
+    got = embedding.embedding_grad(ids, dy, 1009, scale=2.5)
+    check_grad(got, ids, dy, 2.5)
+    assert torch.equal(got, embedding.embedding_grad(ids, dy, 1009, scale=2.5))
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 255, 256, 49152, 65535, 65536, 70001])
+@pytest.mark.parametrize("n", [20000, 40000])
+def test_gradient_of_any_vocabulary_by_several_workgroups(hip_device, vocab, n):
+    """One, two and three passes of the sort over several tiles."""
+    gen = torch.Generator(hip_device).manual_seed(vocab + n)
+    ids = make_ids("random", n, vocab, gen, hip_device, torch.int32)
+    dy = torch.randn(n, 24, device=hip_device, generator=gen)
+    check_grad(embedding.embedding_grad(ids, dy, vocab, dtype=BF16), ids, dy, 1.0)
+
+
+@pytest.mark.parametrize("w", [FP32, BF16])
+@pytest.mark.parametrize("vocab,kind", [(200, "random"), (400, "few"), (70001, "random"), (70001, "same")])
+def test_gradient_added_by_several_workgroups(hip_device, w, vocab, kind):
+    """Added to a buffer with a row stride, and written over it, its rows cleared
+    piece by piece beside the passes."""
+    n = 20011
+    gen = torch.Generator(hip_device).manual_seed(vocab)
+    store = torch.randn(vocab, 50, device=hip_device, generator=gen).to(w)
+    before, out = store.clone(), store[:, 2:45]
+    ids = make_ids(kind, n, vocab, gen, hip_device)
+    ids[0], ids[1], ids[n - 1] = vocab - 1, -100, vocab
+    dy = torch.randn(n, 43, device=hip_device, generator=gen)
+    embedding.embedding_grad(ids, dy, vocab, out=out, accumulate=True)
+    check_grad(out, ids, dy, 1.0, old=before[:, 2:45])
+    assert torch.equal(store[:, :2], before[:, :2]) and torch.equal(store[:, 45:], before[:, 45:])
+    embedding.embedding_grad(ids, dy, vocab, out=out)
+    check_grad(out, ids, dy, 1.0)
+    assert torch.equal(store[:, :2], before[:, :2]) and torch.equal(store[:, 45:], before[:, 45:])
+
+
+@pytest.mark.parametrize("vocab", [200, 3000, 70001])
+def test_several_workgroups_captured_and_replayed(hip_device, vocab):
+    gen = torch.Generator(hip_device).manual_seed(vocab)
+    n = 20000
+    ids = make_ids("random", n, vocab, gen, hip_device)
+    dy = torch.randn(n, 24, device=hip_device, generator=gen)
+    kept = torch.randn(vocab, 24, device=hip_device, generator=gen)
+    old = kept.clone()
+    side = torch.cuda.Stream(hip_device)
+    with torch.cuda.stream(side):
+        embedding.embedding_grad(ids, dy, vocab)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad = embedding.embedding_grad(ids, dy, vocab)
+        embedding.embedding_grad(ids, dy, vocab, out=kept, accumulate=True)
+    for kind in ("padded", "same", "few", "random"):
+        ids.copy_(make_ids(kind, n, vocab, gen, hip_device))
+        dy.normal_(generator=gen)
+        kept.copy_(old)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, embedding.embedding_grad(ids, dy, vocab))
+        assert torch.equal(kept, embedding.embedding_grad(ids, dy, vocab, out=old.clone(), accumulate=True))
+
+
+@pytest.mark.parametrize("vocab", [200, 1009, 70001])
+@pytest.mark.parametrize("kind", ["random", "few", "padded"])
+def test_gradient_of_more_tiles_than_counts_in_lds(hip_device, vocab, kind):
+    """Runs of a frequent id over thousands of units; the passes count the next
+    one's digits in global memory."""
+    n = 530_003
+    gen = torch.Generator(hip_device).manual_seed(vocab)
+    ids = make_ids(kind, n, vocab, gen, hip_device)
+    dy = torch.randn(n, 8, device=hip_device, generator=gen)
+    got = embedding.embedding_grad(ids, dy, vocab)
+    check_grad(got, ids, dy, 1.0)
+    assert torch.equal(got, embedding.embedding_grad(ids, dy, vocab))
