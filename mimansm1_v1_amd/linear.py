@@ -207,7 +207,9 @@ def fused_linear(x, w, bias=None, activation="none", residual=None, out_dtype=No
 class Linear(nn.Linear):
     """``nn.Linear`` (same parameters, state and initialisation) on
     ``fused_linear``: ``forward(x, residual=None)`` is
-    ``act(x weight^T + bias) + residual``."""
+    ``act(x weight^T + bias) + residual``.  The arithmetic is ``fused_linear``'s
+    whatever the parameters' type: fp32 ones enter the product rounded to bf16,
+    under autocast or not, and their gradients come from bf16 operands."""
 
     def __init__(self, in_features, out_features, bias=True, activation="none", device=None, dtype=None):
         super().__init__(in_features, out_features, bias, device=device, dtype=dtype)
