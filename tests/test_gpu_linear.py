@@ -424,3 +424,32 @@ def test_infinite_and_missing_values(hip_device, act, rows):
     if act == "gelu":
         x[rows - 3:, 0] = torch.tensor([-20, -1e4, -3e38], device=hip_device)
         assert not linear.fused_linear(x, w, activation=act, out_dtype=FP32)[rows - 3:].any()
+
+
+@pytest.mark.parametrize("flipped", [False, True])
+@pytest.mark.parametrize("act,k,n", [("none", 64, 4_000_000), ("silu", 40, 3_999_999), ("none", 4_000_000, 64),
+                                     ("silu", 3_999_998, 24)])
+def test_widest_matrices(hip_device, act, k, n, flipped):
+    """The documented limits, forward and backward, where rows lie furthest apart."""
+    check(act, *make(130, k, n, hip_device, 13, flipped=flipped, bias=FP32, residual=FP32))
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("act,n", [("silu", 3_999_000), ("none", 3_999_000), ("none", 1000)])
+def test_strides_up_to_the_bound(hip_device, act, n):
+    """The C entry with fp32 rows of output and residual as far apart as it takes them,
+    where a wave has 128 of them: the values of the contiguous call, nothing else written."""
+    m, k, far = 256, 64, ((1 << 30) - 64) // 127
+    x, w, _, residual = make(m, k, n, hip_device, 15, residual=FP32)
+    want = linear.fused_linear(x, w, activation=act, residual=residual)
+    apart = torch.zeros(m * far, device=hip_device).as_strided((m, far), (far, 1))
+    apart[:, :n] = residual
+    out = torch.full((m * far,), 7.0, device=hip_device).as_strided((m, far), (far, 1))
+    code = linear.ACTIVATIONS[act]
+    keep, ws, nbytes = linear.workspace(linear._product_bytes(m, n, k, linear.ROW, code), hip_device)
+    linear.call("mm1_linear", hip_device, x.data_ptr(), linear.ROW, k, w.data_ptr(), linear.ROW, k, None, 0, code,
+                apart.data_ptr(), 1, far, None, 0, out.data_ptr(), 1, far, ws, nbytes, m, n, k)
+    assert torch.equal(out[:, :n], want)
+    assert bool((out[:, n:] == 7).all())
+    del apart, out
+    torch.cuda.empty_cache()
