@@ -2,10 +2,11 @@
 torch in the same arithmetic (lookup) and against 64-bit sums (gradient)."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from mimansm1_v1_amd import embedding, lm_head
+from mimansm1_v1_amd import _lib, embedding, lm_head
 
 pytestmark = pytest.mark.gpu
 
@@ -382,3 +383,52 @@ def test_gradient_of_more_tiles_than_counts_in_lds(hip_device, vocab, kind):
     got = embedding.embedding_grad(ids, dy, vocab)
     check_grad(got, ids, dy, 1.0)
     assert torch.equal(got, embedding.embedding_grad(ids, dy, vocab))
+
+
+@pytest.mark.parametrize("w", [FP32, BF16])
+def test_rows_past_32_bit_offsets(hip_device, w):
+    """A matrix, and a batch, of more than 2^31 values: lookup and gradient at both ends."""
+    vocab, dim, n = 2_200_003, 1000, 3000
+    gen = torch.Generator(hip_device).manual_seed(6)
+    weight = torch.empty(vocab, dim, device=hip_device, dtype=w).normal_(generator=gen)
+    ids = torch.cat([torch.randint(0, 100, (n // 2,), generator=gen, device=hip_device),
+                     torch.randint(vocab - 1000, vocab, (n - n // 2,), generator=gen, device=hip_device)])
+    assert torch.equal(embedding.embed(ids, weight), weight[ids])
+    dy = torch.randn(n, dim, device=hip_device, generator=gen)
+    grad = embedding.embedding_grad(ids, dy, vocab, out=weight)
+    low, high = grad[:100].clone(), grad[vocab - 1000:].clone()
+    assert not grad[100:vocab - 1000].any()
+    outside = torch.where(ids < 100, ids, -1)
+    check_grad(low, outside, dy, 1.0)
+    check_grad(high, torch.where(ids >= 100, ids - (vocab - 1000), -1), dy, 1.0)
+    del weight, grad
+    small = torch.randn(50, dim, device=hip_device, generator=gen).to(w)
+    many = torch.randint(0, 50, (vocab,), generator=gen, device=hip_device)
+    y = embedding.embed(many, small, out_dtype=BF16)
+    for part in (slice(0, 1000), slice(vocab - 1000, vocab)):
+        assert torch.equal(y[part], small[many[part]].to(BF16))
+    # the sums read rows past 2^31 values: a token counts where its id is in range
+    many[1000:vocab - 1000] = -1
+    got = embedding.embedding_grad(many, y, 50)
+    check_grad(got, torch.cat([many[:1000], many[vocab - 1000:]]), torch.cat([y[:1000], y[vocab - 1000:]]), 1.0)
+    del y
+    torch.cuda.empty_cache()
+
+
+def test_gradient_of_the_most_tokens(hip_device):
+    """2^26 tokens, the most that are taken, a quarter of them the same one, against
+    64-bit sums on the host."""
+    n, vocab = 1 << 26, 70001
+    gen = torch.Generator(hip_device).manual_seed(7)
+    ids = (torch.rand(n, device=hip_device, generator=gen) ** 8 * vocab).int().clamp(max=vocab - 1)
+    dy = torch.randn(n, 1, device=hip_device, generator=gen)
+    got = embedding.embedding_grad(ids, dy, vocab)[:, 0].cpu().numpy()
+    index, terms = ids.cpu().numpy(), dy[:, 0].double().cpu().numpy()
+    want, size = np.bincount(index, terms, vocab), np.bincount(index, np.abs(terms), vocab)
+    count = np.bincount(index, minlength=vocab)
+    assert (np.abs(got - want) <= (count + 3) * 2.0 ** -24 * 1.01 * size).all()
+    more = torch.zeros(n + 1, dtype=torch.int32, device=hip_device)
+    with pytest.raises(_lib.AttnError):
+        embedding.embedding_grad(more, dy[:1].expand(n + 1, 1), vocab)
+    del ids, dy, more
+    torch.cuda.empty_cache()

@@ -257,3 +257,22 @@ def test_a_gradient_given_twice(hip_device):
         assert abs(norm.item() - exact_norm([t, t], 2.0)) <= 1.01 * U * exact_norm([t, t], 2.0)
         check_clipped(clipped, [before, before], exact_norm([t, t], 2.0), 0.5)
     assert torch.equal(t, before)
+
+
+def test_values_past_32_bit_offsets(hip_device):
+    """A tensor of more than 2^32 values, and rows of one that lie further apart."""
+    n = (1 << 32) + 5001
+    t = torch.zeros(n, dtype=BF16, device=hip_device)
+    t[-1], t[5], t[1 << 31] = 3.0, 4.0, 12.0
+    assert grad_clip.grad_norm([t], math.inf).item() == 12 and grad_clip.grad_norm([t]).item() == 13
+    (clipped,), norm = grad_clip.clip_grads([t], 6.5)
+    assert norm.item() == 13 and abs(clipped[-1].item() - 1.5) <= 2.0 ** -7 and abs(clipped[1 << 31].item() - 6) <= 2.0 ** -5
+    assert not clipped[6:1 << 31].any() and not clipped[(1 << 31) + 1:-1].any()
+    del clipped
+    rows = t.as_strided((3, 900), (1 << 31, 1), 4096)
+    rows.fill_(1.0)
+    assert abs(grad_clip.grad_norm([rows]).item() - 2700 ** 0.5) <= 1.01 * U * 2700 ** 0.5
+    grad_clip.clip_grads([rows], 1.0, out=[rows])
+    assert bool(((rows.double() * 2700 ** 0.5 - 1).abs() <= 2.0 ** -8 + 1e-6).all()) and t[5] == 4 and t[4095] == 0
+    del rows, t
+    torch.cuda.empty_cache()
