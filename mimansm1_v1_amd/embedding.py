@@ -61,19 +61,16 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _extent(t):
-    """The bytes [first, last) that a tensor's values lie in (with what lies between them)."""
-    last = sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride())) + 1
-    return t.data_ptr(), t.data_ptr() + last * t.element_size()
+def _span(t):
+    """The bytes from a tensor's first value to behind its last."""
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
 def _shares(out, t):
-    """Whether `out`, rows of values, may share memory with `t`: their extents meet
+    """Whether `out`, rows of values, may share memory with `t`: their spans meet
     and they are not different columns of rows equally far apart."""
-    if not t.numel():
-        return False
-    (a0, a1), (b0, b1) = _extent(out), _extent(t)
-    if a1 <= b0 or b1 <= a0:
+    a0, b0 = out.data_ptr(), t.data_ptr()
+    if (b0 >= a0 + _span(out) if b0 >= a0 else a0 >= b0 + _span(t)) or not t.numel():
         return False
     pitch, width = out.stride(0) * out.element_size(), out.shape[1] * out.element_size()
     steps = [(n, s) for n, s in zip(t.shape, t.stride()) if n > 1]
